@@ -324,7 +324,7 @@ def _own_plan(s, c):
 def _own_keep(s, c):
     from flash_attention_b200 import paged_cache
 
-    lens = paged_cache.keep_tree_path(s["caches"], s["lens"], s["path"], c["nodes"], block_table=s["block_table"])
+    lens = paged_cache.keep_tree_path(s["caches"].unbind(0), s["lens"], s["path"], c["nodes"], block_table=s["block_table"])
     return {"caches": s["caches"], "lens": lens}
 
 
