@@ -297,9 +297,11 @@ __global__ void __launch_bounds__(160, D > 128 ? 1 : 2) decode_kernel(const __gr
         const T* vn = reinterpret_cast<const T*>(a.vnew.ptr) + b * a.vnew.stride_b + hk * a.vnew.stride_h;
         const int64_t slab = pages ? pages[L / a.page_block_size] : cb;
         const int64_t srow = pages ? L % a.page_block_size : L;
+        // (a page or slot that is not there takes nothing, as in kvcache_prep.cu: its rows read as zeros)
+        const int n = slab >= 0 && slab < a.batch_cache ? 2 * (D / 8) : 0;
         T* kg = reinterpret_cast<T*>(a.kcache.ptr) + slab * a.kcache.stride_b + srow * a.kcache.stride_s + hk * a.kcache.stride_h;
         T* vg = reinterpret_cast<T*>(a.vcache.ptr) + slab * a.vcache.stride_b + srow * a.vcache.stride_s + hk * a.vcache.stride_h;
-        for (int c = tid; c < 2 * (D / 8); c += 128) {
+        for (int c = tid; c < n; c += 128) {
           const bool is_v = c >= D / 8;
           const int d0 = (is_v ? c - D / 8 : c) * 8;
           uint4 val = is_v ? *reinterpret_cast<const uint4*>(vn + d0)

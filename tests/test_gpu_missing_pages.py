@@ -1,0 +1,56 @@
+"""Block-table entries and slot numbers that name no page of the cache, one token per sequence: the token is dropped, the rows read as zeros, and
+nothing outside the cache is read or written.  The caches are the middle of larger allocations, so that a stray address lands in pages that are looked at."""
+import pytest
+import torch
+
+import flash_attention_b200 as fa
+from flash_attention_b200 import _lib
+from oracle import tree_oracle as TO
+
+pytestmark = pytest.mark.gpu
+GUARD, POOL, BATCH, PAGE = 6, 12, 4, 64
+
+
+def guarded(rows, heads_k, dim, g):
+    """A pool with GUARD pages in front of it and behind it, which hold values that would show in any result."""
+    whole = torch.randn(GUARD + POOL + GUARD, rows, heads_k, dim, generator=g).bfloat16()
+    whole[:GUARD], whole[GUARD + POOL:] = 1000.0, -1000.0
+    return whole.cuda()
+
+
+def check(out, lse, q, kc, vc, lens, **kw):
+    """A token that sees itself and what is in front of it is a tree of one node."""
+    sees = torch.ones(1, 1, 1, dtype=torch.bool)
+    o, l, to, tl = TO.tree_attention(q.cpu(), kc.cpu(), vc.cpu(), sees, lens.cpu(), **kw)
+    assert ((out.double().cpu() - o).abs() <= to).all()
+    assert ((lse.double().cpu() - l).abs() <= tl).all()
+
+
+# one token in the fused kernel (dims 64 and 128), behind kvcache_prep on the tensor cores (24 rows per KV head)
+@pytest.mark.parametrize("heads,heads_k,dim,path", [(8, 2, 128, "decode"), (4, 4, 64, "decode"), (48, 2, 128, "kvcache_prep+fwd_tc")])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("paged", [True, False])
+def test_one_token(heads, heads_k, dim, path, splits, paged):
+    g = torch.Generator().manual_seed(dim + heads)
+    rows = PAGE if paged else 3 * PAGE
+    whole = [guarded(rows, heads_k, dim, g) for _ in range(2)]
+    was = [w.clone() for w in whole]
+    kc, vc = (w[GUARD:GUARD + POOL] for w in whole)
+    lens = torch.tensor([70, 64, 130, 0], dtype=torch.int32)
+    q = torch.randn(BATCH, 1, heads, dim, generator=g).bfloat16()
+    k, v = (torch.randn(BATCH, 1, heads_k, dim, generator=g).bfloat16() for _ in range(2))
+    if paged:
+        table = torch.tensor([[3, -1, 5], [7, POOL, 0], [1, 2, POOL + GUARD - 1], [-GUARD, 4, 6]], dtype=torch.int32)
+        place, kw = {}, dict(block_table=table)
+    else:
+        slots = torch.tensor([-1, 3, POOL, -GUARD], dtype=torch.int32)
+        place, kw = {1: (3, 64)}, dict(cache_batch_idx=slots)
+    out, lse = fa.flash_attn_with_kvcache(q.cuda(), kc, vc, k.cuda(), v.cuda(), cache_seqlens=lens.cuda(), causal=True, num_splits=splits, return_softmax_lse=True,
+                                          **{n: t.cuda() for n, t in kw.items()})
+    torch.cuda.synchronize()
+    assert _lib.last_path().startswith(path), _lib.last_path()
+    for w, x, new in zip(whole, was, (k, v)):
+        for b, (slab, row) in place.items():
+            x[GUARD + slab, row] = new[b, 0].cuda()
+        assert torch.equal(w, x)
+    check(out, lse, q, kc, vc, lens, **kw)
