@@ -10,7 +10,7 @@
 #include "fa_common.cuh"
 
 namespace fa {
-int fwd_generic(const FaFwdArgs& a, cudaStream_t st);
+int fwd_generic(const FaFwdArgs& a, int64_t slabs, cudaStream_t st);
 int bwd_pre(const FaBwdArgs& a, int zero_dq, cudaStream_t st);
 int bwd_post(const FaBwdArgs& a, cudaStream_t st);
 int bwd_generic_main(const FaBwdArgs& a, cudaStream_t st);
@@ -293,7 +293,7 @@ int fa_fwd(const FaFwdArgs* a, fa_stream_t stream) {
     rc = fa::fwd_tc(*a, st);
   } else {
     g_last_path = a->num_splits > 1 ? "fwd_generic+combine" : "fwd_generic";
-    rc = fa::fwd_generic(*a, st);
+    rc = fa::fwd_generic(*a, 0, st);
   }
   if (rc) return rc;
   if (a->num_splits > 1)
@@ -473,7 +473,7 @@ int fa_fwd_kvcache(const FaKvcacheArgs* a, fa_stream_t stream) {
     return fa::decode_run(c, splits, st, true, a->knew.ptr ? a->seqlen_new : 0, a->window_right == 0);
   }
   const FaFwdArgs f = cache_fwd_args(*a, splits);
-  rc = tc ? fa::fwd_tc_cache(f, a->batch_cache, st) : fa::fwd_generic(f, st);
+  rc = tc ? fa::fwd_tc_cache(f, a->batch_cache, st) : fa::fwd_generic(f, a->batch_cache, st);
   if (rc) return rc;
   if (splits > 1)
     return fa::combine(a->out_accum, a->lse_accum, a->out, a->softmax_lse, a->seqlen_q, splits, a->batch, a->heads,

@@ -28,8 +28,8 @@ __device__ __forceinline__ void load_tile_64(T* s, const T* g, int64_t row_strid
   }
 }
 
-// TREE: the query rows are the nodes of a tree, the last seqlen_q keys of a KV cache of `slabs` pages or sequence slots (TreeMask).  Pages that the pool
-// does not have read as zeros, as they do through a tensor map.
+// slabs: pages or sequence slots of a KV cache, 0 for other calls.  Those that the cache does not have read as zeros, as they do through a tensor map.
+// TREE: the query rows are the nodes of a tree, the last seqlen_q keys of the cache (TreeMask).
 template <typename T, int DP, bool TREE>
 __global__ void __launch_bounds__(128) fwd_generic_kernel(const __grid_constant__ FaFwdArgs p, const TreeMask tree, int64_t slabs) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -50,12 +50,13 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const __grid_constant_
     node0 = min(max(si.sk - p.seqused_k_extra, 0), p.seqlen_k);
     si.sk = min(node0 + p.seqused_k_extra, p.seqlen_k);
   }
+  if (slabs > 0) si.sk = min(si.sk, p.seqlen_k);  // (a length past the capacity sees the whole cache)
   const int m0 = blockIdx.x * GF_BM;
   if (m0 >= si.sq) return;
   const int D = p.head_dim;
   const T* qg = reinterpret_cast<const T*>(p.q.ptr) + si.q_batch * p.q.stride_b + si.q_row0 * p.q.stride_s +
                 (int64_t)h * p.q.stride_h;
-  const bool no_slab = TREE && !p.block_table && (si.k_batch < 0 || si.k_batch >= slabs);
+  const bool no_slab = slabs > 0 && !p.block_table && (si.k_batch < 0 || si.k_batch >= slabs);
   const int64_t kbatch = p.block_table || no_slab ? 0 : si.k_batch;  // paged: the page offset is added per tile
   const T* kg = reinterpret_cast<const T*>(p.k.ptr) + kbatch * p.k.stride_b + si.k_row0 * p.k.stride_s +
                 (int64_t)hk * p.k.stride_h;
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const __grid_constant_
       int64_t page = p.block_table[(int64_t)b * p.block_table_stride + n0 / p.page_block_size];
       const int r0 = n0 % p.page_block_size;
       int r_end = r0 + (si.sk - n0);
-      if (TREE && (page < 0 || page >= slabs)) page = 0, r_end = 0;  // (no row of the tile is read)
+      if (slabs > 0 && (page < 0 || page >= slabs)) page = 0, r_end = 0;  // (no row of the tile is read)
       load_tile_64<T, DP>(sK, kg + page * p.k.stride_b, p.k.stride_s, r0, r_end, D, tid);
       load_tile_64<T, DP>(sV, vg + page * p.v.stride_b, p.v.stride_s, r0, r_end, D, tid);
     } else {
@@ -324,7 +325,7 @@ static int dispatch_fwd_generic(const FaFwdArgs& a, int64_t slabs, const TreeMas
 static int run_fwd_generic(const FaFwdArgs& a, int64_t slabs, const TreeMask* tree, cudaStream_t st) {
   return a.dtype == FA_DTYPE_BF16 ? dispatch_fwd_generic<__nv_bfloat16>(a, slabs, tree, st) : dispatch_fwd_generic<__half>(a, slabs, tree, st);
 }
-int fwd_generic(const FaFwdArgs& a, cudaStream_t st) { return run_fwd_generic(a, 0, nullptr, st); }
+int fwd_generic(const FaFwdArgs& a, int64_t slabs, cudaStream_t st) { return run_fwd_generic(a, slabs, nullptr, st); }
 int fwd_generic_tree(const FaFwdArgs& a, int64_t slabs, const TreeMask& tree, cudaStream_t st) { return run_fwd_generic(a, slabs, &tree, st); }
 
 }  // namespace fa

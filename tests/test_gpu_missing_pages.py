@@ -26,8 +26,11 @@ def check(out, lse, q, kc, vc, lens, **kw):
     assert ((lse.double().cpu() - l).abs() <= tl).all()
 
 
-# one token in the fused kernel (dims 64 and 128), behind kvcache_prep on the tensor cores (24 rows per KV head)
-@pytest.mark.parametrize("heads,heads_k,dim,path", [(8, 2, 128, "decode"), (4, 4, 64, "decode"), (48, 2, 128, "kvcache_prep+fwd_tc")])
+# one token in the fused kernel (dims 64 and 128), behind kvcache_prep on the tensor cores (24 rows per KV head) and in the any-shape kernel
+PATHS = [(8, 2, 128, "decode"), (4, 4, 64, "decode"), (48, 2, 128, "kvcache_prep+fwd_tc"), (8, 2, 96, "kvcache_prep+fwd_generic")]
+
+
+@pytest.mark.parametrize("heads,heads_k,dim,path", PATHS)
 @pytest.mark.parametrize("splits", [1, 3])
 @pytest.mark.parametrize("paged", [True, False])
 def test_one_token(heads, heads_k, dim, path, splits, paged):
@@ -54,3 +57,24 @@ def test_one_token(heads, heads_k, dim, path, splits, paged):
             x[GUARD + slab, row] = new[b, 0].cuda()
         assert torch.equal(w, x)
     check(out, lse, q, kc, vc, lens, **kw)
+
+
+@pytest.mark.parametrize("heads,heads_k,dim,path", PATHS)
+@pytest.mark.parametrize("splits", [1, 3])
+def test_lengths_past_the_capacity(heads, heads_k, dim, path, splits):
+    """Such a sequence sees the whole cache; its token is dropped."""
+    g = torch.Generator().manual_seed(dim + heads)
+    whole = [guarded(PAGE, heads_k, dim, g) for _ in range(2)]
+    was = [w.clone() for w in whole]
+    kc, vc = (w[GUARD:GUARD + POOL] for w in whole)
+    table = torch.randperm(POOL, generator=g).view(BATCH, 3).int()
+    lens = torch.tensor([192, 500, 10, 191], dtype=torch.int32)
+    q = torch.randn(BATCH, 1, heads, dim, generator=g).bfloat16()
+    k, v = (torch.randn(BATCH, 1, heads_k, dim, generator=g).bfloat16() for _ in range(2))
+    out, lse = fa.flash_attn_with_kvcache(q.cuda(), kc, vc, k.cuda(), v.cuda(), cache_seqlens=lens.cuda(), causal=True, num_splits=splits, return_softmax_lse=True,
+                                          block_table=table.cuda())
+    assert _lib.last_path().startswith(path), _lib.last_path()
+    for w, x, new in zip(whole, was, (k, v)):
+        x[GUARD + int(table[2, 0]), 10], x[GUARD + int(table[3, 2]), 63] = new[2, 0].cuda(), new[3, 0].cuda()
+        assert torch.equal(w, x)
+    check(out, lse, q, kc, vc, lens, block_table=table)
