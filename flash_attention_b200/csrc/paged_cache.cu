@@ -268,44 +268,42 @@ __global__ void __launch_bounds__(128) keep_path_kernel(const __grid_constant__ 
   __shared__ int count;
   const int b = blockIdx.x, tid = threadIdx.x;
   const int L = a.cache_seqlens[b];
+  auto place = [&](int64_t row) -> int64_t {
+    if (row < 0 || row >= a.seqlen_cache) return -1;
+    int64_t slab = a.cache_batch_idx ? a.cache_batch_idx[b] : b;
+    int64_t r = row;
+    if (a.block_table) {
+      const int q = (int)p.page.div((uint32_t)row);
+      slab = a.block_table[b * a.table_stride + q];
+      r = row - (int64_t)q * a.page_block_size;
+    }
+    return slab < 0 || slab >= a.batch_cache ? -1 : slab * a.stride_b + r * a.stride_s;
+  };
   if (tid < 32) {
-    int n = a.depth;
+    int n = 0;
     for (int i0 = 0; i0 < a.depth; i0 += 32) {
       const int i = i0 + tid;
       const int node = i < a.depth ? a.path[b * a.path_stride + i] : -1, last = i > 0 && i < a.depth ? a.path[b * a.path_stride + i - 1] : -1;
-      const uint32_t ends = __ballot_sync(0xffffffffu, !(node > last && node >= 0 && node < a.nodes));
-      if (ends) {
-        n = i0 + __ffs(ends) - 1;
-        break;
+      bool on = node > last && node >= 0 && node < a.nodes;
+      int64_t src = -1, dst = -1;
+      if (on && have_caches) {  // a node whose row, or the row it would move to, is not there was never stored: it ends the path as well
+        src = place((int64_t)L + node), dst = place((int64_t)L + i);
+        on = src >= 0 && dst >= 0;
       }
+      const uint32_t ends = __ballot_sync(0xffffffffu, !on);
+      const int more = ends ? __ffs(ends) - 1 : 32;
+      if (tid < more) keep_smem[2 * i] = node != i ? src : -1, keep_smem[2 * i + 1] = dst;
+      n += more;
+      if (ends) break;
     }
     if (tid == 0) {
-      count = n = min(n, a.depth);
+      count = n;
       if (blockIdx.y == 0 && blockIdx.z == 0 && a.new_seqlens) a.new_seqlens[b] = L + n;
     }
   }
   __syncthreads();
   const int n = count;
   if (!have_caches) return;
-  auto place = [&](int row) -> int64_t {
-    if (row < 0 || row >= a.seqlen_cache) return -1;
-    int64_t slab = a.cache_batch_idx ? a.cache_batch_idx[b] : b;
-    int r = row;
-    if (a.block_table) {
-      const int q = (int)p.page.div((uint32_t)row);
-      slab = a.block_table[b * a.table_stride + q];
-      r = row - q * a.page_block_size;
-    }
-    return slab < 0 || slab >= a.batch_cache ? -1 : slab * a.stride_b + r * a.stride_s;
-  };
-  for (int i = tid; i < n; i += 128) {
-    const int node = a.path[b * a.path_stride + i];
-    const int64_t src = place(L + node), dst = place(L + i);
-    const bool moves = node != i && src >= 0 && dst >= 0;
-    keep_smem[2 * i] = moves ? src : -1;
-    keep_smem[2 * i + 1] = dst;
-  }
-  __syncthreads();
   constexpr int E = sizeof(V) / 2;
   uint16_t* cache = reinterpret_cast<uint16_t*>(p.caches[blockIdx.y]);
   for (int c = blockIdx.z * 128 + tid; c < p.pieces; c += gridDim.z * 128) {

@@ -75,6 +75,7 @@ def keep_tree_path(caches: Union[Sequence[torch.Tensor], torch.Tensor], cache_se
     caches: K and V caches of any number of layers, of one shape, dtype and layout, paged with block_table, else a slab per sequence; or all of
         them as one tensor with the caches along its first dimension.
     path: (batch, longest) int32, the accepted nodes of each sequence from the top: each later than the one before and below `nodes`; any other
-        value ends the path (pad with -1).  Rows of the tree that are not on the path hold anything afterwards.
+        value ends the path (pad with -1), and so does a node that is not in the caches, its row being past their capacity or in a page or slot
+        that is not there.  Rows of the tree that are not on the path hold anything afterwards.
     Returns cache_seqlens plus the number of accepted nodes, (batch,) int32.  Sequences must not share the rows that move."""
     return _ext._glue.keep_path(caches, cache_seqlens, path, nodes, block_table, cache_batch_idx)

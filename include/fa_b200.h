@@ -336,7 +336,8 @@ int fa_pack_tree_mask(const uint8_t* mask, int64_t stride_b, int64_t stride_i, i
                       fa_stream_t stream);
 
 /* The nodes on path[b, 0..) (each after the one before, ended by any other value or the row's end) move to rows cache_seqlens[b] + 0, 1, ... of each of
-   n_caches caches of the same shape and strides (16-bit elements); new_seqlens[b] = cache_seqlens[b] + their number. */
+   n_caches caches of the same shape and strides (16-bit elements); new_seqlens[b] = cache_seqlens[b] + their number.  A node whose row, or the row
+   it would move to, is past the capacity or in a page or slot that is not there was never stored: it ends the path too. */
 typedef struct FaKeepArgs {
   void* const* caches;           /* host array */
   int32_t n_caches;

@@ -168,14 +168,16 @@ def pack_words(sees):
 
 
 def keep(cache_of, lens, path, nodes, cap):
-    """cache_of(b, row) -> key of a place; returns the moves [(from, to)] of every sequence in order, and the new lengths."""
+    """cache_of(b, row) -> key of a place, None for one that is not there; returns the moves [(from, to)] of every sequence in order, and the new lengths.  A
+    path ends at the first node that does not go on, or whose row, or the row it moves to, is not there."""
+    there = lambda b, row: 0 <= row < cap and cache_of(b, row) is not None  # noqa: E731
     moves, new = [], []
     for b, (length, steps) in enumerate(zip(lens, path)):
         last, n = -1, 0
         for node in steps:
-            if not (last < node < nodes):
+            if not (last < node < nodes) or not there(b, length + node) or not there(b, length + n):
                 break
-            if node != n and length + node < cap:
+            if node != n:
                 moves.append((cache_of(b, length + node), cache_of(b, length + n)))
             last, n = node, n + 1
         new.append(length + n)

@@ -1,0 +1,73 @@
+"""keep_tree_path where the accepted nodes, or the rows they move to, are not in the caches: the path ends there, in the caches and in the lengths."""
+import pytest
+import torch
+
+from flash_attention_b200 import paged_cache as pc
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def cache(*shape):
+    return torch.randint(-1000, 1000, shape, device="cuda").to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_node_past_the_capacity_ends_the_path(paged):
+    """192 rows, 185 of them taken: nodes 0 to 6 were stored, node 10 was not."""
+    table = ints([[2, 0, 1]]) if paged else None
+    c = cache(3, 64, 2, 64) if paged else cache(1, 192, 2, 64)
+    rows = lambda: torch.cat([c[p] for p in (2, 0, 1)]) if paged else c[0]  # noqa: E731
+    was = rows().clone()
+    for path, kept, moves in (([0, 10], 186, {}), ([10], 185, {}), ([2, 6, 7], 187, {185: 187, 186: 191}), ([0, 1, 2, 3, 4, 5, 6, 7], 192, {})):
+        for t, x in zip((c[2], c[0], c[1]) if paged else (c[0][:64], c[0][64:128], c[0][128:]), was.split(64)):
+            t.copy_(x)
+        assert pc.keep_tree_path([c], ints([185]), ints([path]), 12, block_table=table).tolist() == [kept]
+        want = was.clone()
+        for to, at in moves.items():
+            want[to] = was[at]
+        assert torch.equal(rows(), want)
+
+
+def test_lengths_at_and_past_the_capacity_and_below_zero():
+    c = cache(4, 64, 2, 64)
+    was = c.clone()
+    assert pc.keep_tree_path([c], ints([64, 100, -3, 2 ** 31 - 2]), ints([[0, 1]] * 4), 3).tolist() == [64, 100, -3, 2 ** 31 - 2]
+    assert torch.equal(c, was)
+
+
+def test_pages_and_slots_that_are_not_there():
+    """The page of a node, or of the row it would move to."""
+    c = cache(6, 64, 2, 64)
+    was = c.clone()
+    table = ints([[3, -1, 4], [-1, 5, 0], [0, 6, 1], [1, 2, 3]])
+    lens, path = ints([60, 62, 62, 62]), ints([[0, 3, 5], [1, 2, 3], [0, 1, 2], [0, 2, 3]])
+    # 0: rows 60, 63, then a row of the missing page; 1: its first target is missing; 2: rows 62, 63, then a missing one; 3: all there
+    assert pc.keep_tree_path([c], lens, path, 8, block_table=table).tolist() == [62, 62, 64, 65]
+    want = was.clone()
+    want[3, 61] = was[3, 63]
+    want[1, 63], want[2, 0] = was[2, 0], was[2, 1]
+    assert torch.equal(c, want)
+    c.copy_(was)
+    assert pc.keep_tree_path([c], ints([10, 10, 10]), ints([[1, 2]] * 3), 8, cache_batch_idx=ints([5, -1, 6])).tolist() == [12, 10, 10]
+    want = was.clone()
+    want[5, 10], want[5, 11] = was[5, 11], was[5, 12]
+    assert torch.equal(c, want)
+
+
+@pytest.mark.parametrize("depth", [31, 32, 33, 64, 65, 100])
+def test_long_paths_that_end_at_the_capacity(depth):
+    """The end in the first, the second and the third group of 32 nodes, and at their borders."""
+    nodes = 2 * depth
+    for room in (1, depth, 2 * depth - 1, 2 * depth):
+        c = cache(1, 20 + room, 1, 8)
+        was = c.clone()
+        path = list(range(1, nodes, 2))
+        kept = sum(node < room for node in path)
+        assert pc.keep_tree_path([c], ints([20]), ints([path]), nodes).tolist() == [20 + kept]
+        want = was.clone()
+        want[0, 20:20 + kept] = was[0, 21:21 + 2 * kept:2]
+        assert torch.equal(c, want)
