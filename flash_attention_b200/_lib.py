@@ -145,7 +145,7 @@ class FaKeepArgs(C.Structure):
         ("cache_seqlens", c_vp), ("cache_batch_idx", c_vp),
         ("block_table", c_vp), ("table_stride", c_i64), ("page_block_size", c_i32),
         ("path", c_vp), ("path_stride", c_i64), ("depth", c_i32), ("nodes", c_i32),
-        ("new_seqlens", c_vp),
+        ("new_seqlens", c_vp), ("seqlens", c_vp),
     ]
 
 

@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(128) keep_path_kernel(const __grid_constant__ 
   __shared__ int count;
   const int b = blockIdx.x, tid = threadIdx.x;
   const int L = a.cache_seqlens[b];
+  const int64_t end = a.seqlens ? a.seqlens[b] : INT64_MAX;  // first row that is not the sequence's
   auto place = [&](int64_t row) -> int64_t {
     if (row < 0 || row >= a.seqlen_cache) return -1;
     int64_t slab = a.cache_batch_idx ? a.cache_batch_idx[b] : b;
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(128) keep_path_kernel(const __grid_constant__ 
     for (int i0 = 0; i0 < a.depth; i0 += 32) {
       const int i = i0 + tid;
       const int node = i < a.depth ? a.path[b * a.path_stride + i] : -1, last = i > 0 && i < a.depth ? a.path[b * a.path_stride + i - 1] : -1;
-      bool on = node > last && node >= 0 && node < a.nodes;
+      bool on = node > last && node >= 0 && node < a.nodes && (int64_t)L + node < end;
       int64_t src = -1, dst = -1;
       if (on && have_caches) {  // a node whose row, or the row it would move to, is not there was never stored: it ends the path as well
         src = place((int64_t)L + node), dst = place((int64_t)L + i);

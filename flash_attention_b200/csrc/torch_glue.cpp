@@ -701,12 +701,14 @@ Tensor pack_tree_mask(const Tensor& mask) {
 }
 
 // keep_path: lengths with the accepted nodes
-Tensor keep_path(const py::object& given, const Tensor& lens, const Tensor& path, int64_t nodes, const MaybeTensor& table, const MaybeTensor& batch_idx) {
+Tensor keep_path(const py::object& given, const Tensor& lens, const Tensor& path, int64_t nodes, const MaybeTensor& table, const MaybeTensor& batch_idx,
+                 const MaybeTensor& seqlens) {
   require(is_type(lens, at::kInt, 1) && lens.is_contiguous(), "cache_seqlens must be int32, contiguous, one per sequence");
   const int64_t batch = lens.size(0);
   require(is_type(path, at::kInt, 2) && path.size(0) == batch && (path.size(1) <= 1 || path.stride(1) == 1),
           "path must be int32 of shape (batch, longest path) with contiguous last dimension");
   require(nodes >= 0 && path.size(1) <= 12288 && fits({batch, nodes}), "a path has at most 12288 nodes");
+  if (seqlens) require(is_type(*seqlens, at::kInt, 1) && seqlens->size(0) == batch && seqlens->is_contiguous(), "seqlens must be int32, contiguous, one per sequence");
   FaKeepArgs a = {};
   a.heads_k = a.head_dim = 1;
   std::vector<void*> ptrs;
@@ -757,7 +759,7 @@ Tensor keep_path(const py::object& given, const Tensor& lens, const Tensor& path
     a.stride_b = c.stride(at), a.stride_s = c.stride(at + 1), a.stride_h = c.stride(at + 2);
     a.batch_cache = c.size(at), a.heads_k = c.size(at + 2), a.head_dim = c.size(at + 3);
   }
-  require_device({&lens, &path, maybe(table), maybe(batch_idx), some ? &first : nullptr});
+  require_device({&lens, &path, maybe(table), maybe(batch_idx), maybe(seqlens), some ? &first : nullptr});
   if (!at)
     for (size_t i = 1; i < ptrs.size(); ++i) require_device({&lens, &THPVariable_Unpack(PySequence_Fast_ITEMS(given.ptr())[i])});
   const c10::cuda::CUDAGuard guard(lens.device());
@@ -765,6 +767,7 @@ Tensor keep_path(const py::object& given, const Tensor& lens, const Tensor& path
   a.caches = ptrs.data(), a.n_caches = to_i32(ptrs.size(), "number of caches");
   a.batch = batch, a.seqlen_cache = cap, a.cache_seqlens = i32(lens), a.new_seqlens = i32(out);
   if (batch_idx) a.cache_batch_idx = i32(*batch_idx);
+  if (seqlens) a.seqlens = i32(*seqlens);
   if (table) a.block_table = i32(*table), a.table_stride = table->stride(0), a.page_block_size = page > 0 ? page : 1;
   a.path = i32(path), a.path_stride = path.stride(0), a.depth = path.size(1), a.nodes = nodes;
   check(fa_keep_path(&a, stream_of(lens)), "keep_tree_path");

@@ -149,8 +149,7 @@ class PagedInferenceParams:
     def accept(self, path: torch.Tensor, nodes: int):
         """Keeps the accepted path of every tree of the step (paged_cache.keep_tree_path) and gives the other nodes' pages back.  A sequence that had no
         room for its tree keeps nothing of it."""
-        path = torch.where((self.seqlens > self._before)[:, None], path, -1)
-        kept = paged_cache.keep_tree_path(self.caches.flatten(0, 1), self._before, path, nodes, block_table=self.block_table)
+        kept = paged_cache.keep_tree_path(self.caches.flatten(0, 1), self._before, path, nodes, block_table=self.block_table, seqlens=self.seqlens)
         paged_cache.release_pages(self.block_table, self.seqlens, kept, self.free_pages, self.num_free, self.page_block_size)
         self.lengths = kept
 

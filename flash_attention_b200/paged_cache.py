@@ -9,8 +9,13 @@ block_table[b, j // page_block_size]; see flash_attn_with_kvcache) with drafted 
     each layer:  q = rotary_axes_to_cache(q, k, v, cos, sin, positions, (pairs,), slots, k_cache, v_cache)
                  out = flash_attn_tree_with_kvcache(q, k_cache, v_cache, words, lens, block_table=block_table)
     the program picks the accepted path of each tree
-    kept = keep_tree_path(all_caches, lens, path, nodes, block_table=block_table)
+    kept = keep_tree_path(all_caches, lens, path, nodes, block_table=block_table, seqlens=seqlens)
     release_pages(block_table, seqlens, kept, free_pages, num_free, page_block_size);  lens = kept
+
+A sequence that had no room (seqlens == lens) has no slots, so that rotary_axes_to_cache stores nothing of it, and given seqlens, keep_tree_path keeps nothing
+of it.  What attention says about it means nothing: the table's entries behind its last page are not its own.  Calls that store tokens by the table
+(k and v of the attention calls) must not find them there: give those torch.where((seqlens > lens)[:, None], block_table, -1), where
+-1 names no page, which is neither read nor written.
 
 Not in this version of the reference, whose caches are one slab per sequence.
 """
@@ -69,7 +74,7 @@ def pack_tree_mask(mask):
 
 
 def keep_tree_path(caches: Union[Sequence[torch.Tensor], torch.Tensor], cache_seqlens, path, nodes: int, block_table: Optional[torch.Tensor] = None,
-                   cache_batch_idx: Optional[torch.Tensor] = None):
+                   cache_batch_idx: Optional[torch.Tensor] = None, seqlens: Optional[torch.Tensor] = None):
     """After verification: the accepted nodes' rows move up behind the tokens in front of the tree, in all caches, in place.
 
     caches: K and V caches of any number of layers, of one shape, dtype and layout, paged with block_table, else a slab per sequence; or all of
@@ -77,5 +82,7 @@ def keep_tree_path(caches: Union[Sequence[torch.Tensor], torch.Tensor], cache_se
     path: (batch, longest) int32, the accepted nodes of each sequence from the top: each later than the one before and below `nodes`; any other
         value ends the path (pad with -1), and so does a node that is not in the caches, its row being past their capacity or in a page or slot
         that is not there.  Rows of the tree that are not on the path hold anything afterwards.
+    seqlens: (batch,) int32, the lengths with the trees as reserve_pages gave them: a node whose row is not below ends the path.  Needed where a sequence may
+        have had no room: what its table names behind its last page may be other sequences'.
     Returns cache_seqlens plus the number of accepted nodes, (batch,) int32.  Sequences must not share the rows that move."""
-    return _ext._glue.keep_path(caches, cache_seqlens, path, nodes, block_table, cache_batch_idx)
+    return _ext._glue.keep_path(caches, cache_seqlens, path, nodes, block_table, cache_batch_idx, seqlens)

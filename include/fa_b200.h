@@ -337,7 +337,8 @@ int fa_pack_tree_mask(const uint8_t* mask, int64_t stride_b, int64_t stride_i, i
 
 /* The nodes on path[b, 0..) (each after the one before, ended by any other value or the row's end) move to rows cache_seqlens[b] + 0, 1, ... of each of
    n_caches caches of the same shape and strides (16-bit elements); new_seqlens[b] = cache_seqlens[b] + their number.  A node whose row, or the row
-   it would move to, is past the capacity or in a page or slot that is not there was never stored: it ends the path too. */
+   it would move to, is past the capacity or in a page or slot that is not there was never stored: it ends the path too, and so does one whose row is not
+   below seqlens[b] where those are given. */
 typedef struct FaKeepArgs {
   void* const* caches;           /* host array */
   int32_t n_caches;
@@ -352,6 +353,7 @@ typedef struct FaKeepArgs {
   int64_t path_stride;
   int32_t depth, nodes;
   int32_t* new_seqlens;
+  const int32_t* seqlens;        /* (batch) lengths with the trees (fa_reserve_pages), or NULL */
 } FaKeepArgs;
 int fa_keep_path(const FaKeepArgs* args, fa_stream_t stream);
 

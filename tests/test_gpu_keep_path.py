@@ -1,4 +1,5 @@
-"""keep_tree_path where the accepted nodes, or the rows they move to, are not in the caches: the path ends there, in the caches and in the lengths."""
+"""keep_tree_path where the accepted nodes, or the rows they move to, are not in the caches or not the sequence's: the path ends there, in the caches and
+in the lengths."""
 import pytest
 import torch
 
@@ -71,3 +72,31 @@ def test_long_paths_that_end_at_the_capacity(depth):
         want = was.clone()
         want[0, 20:20 + kept] = was[0, 21:21 + 2 * kept:2]
         assert torch.equal(c, want)
+
+
+def test_a_sequence_that_had_no_room_leaves_the_others_pages_alone():
+    """The second sequence gets no page; what its table names behind its own page belongs to the first one and to nobody."""
+    c = cache(5, 64, 2, 64)
+    table, lens = ints([[3, 1], [2, 3]]), ints([60, 61])
+    free, num = ints([4, 0]), ints([1, 0])  # the stack's first entry: one page for two that want one
+    slots, _, _, seqlens = pc.reserve_pages(table, lens, 8, free, num, 64)
+    assert seqlens.tolist() == [68, 61] and table.tolist() == [[3, 4], [2, 3]] and slots[8:].tolist() == [-1] * 8
+    was = c.clone()
+    path = ints([[1, 4, 5], [1, 4, 5]])
+    kept = pc.keep_tree_path([c], lens, path, 8, block_table=table, seqlens=seqlens)
+    want = was.clone()
+    want[3, 60], want[3, 61], want[3, 62] = was[3, 61], was[4, 0], was[4, 1]
+    assert kept.tolist() == [63, 61] and torch.equal(c, want)
+    # lengths in the middle of a path, and without caches
+    assert pc.keep_tree_path([], lens, path, 8, seqlens=ints([65, 62])).tolist() == [62, 61]
+    # tokens stored by the call: not with a table that names no page for it
+    import flash_attention_b200 as fa
+
+    q, k = torch.randn(2, 8, 4, 64, device="cuda").bfloat16(), torch.randn(2, 8, 2, 64, device="cuda").bfloat16()
+    words = pc.pack_tree_mask(torch.ones(1, 8, 8, dtype=torch.bool, device="cuda"))
+    kc, vc = c.clone(), c.clone()
+    mine = torch.where((seqlens > lens)[:, None], table, -1)
+    fa.flash_attn_tree_with_kvcache(q, kc, vc, words, lens, k=k, v=k, block_table=mine)
+    want = c.clone()
+    want[3, 60:64], want[4, :4] = k[0, :4], k[0, 4:]
+    assert torch.equal(kc, want) and torch.equal(vc, want)
