@@ -134,17 +134,21 @@ class PagedInferenceParams:
 
     def begin(self, tokens: int):
         """Room for `tokens` more tokens of every sequence.  slots, positions (batch, tokens) and seqlens (the lengths with them; a sequence
-        that gets no room keeps its length, and its tokens have no slot) are what the layers take."""
+        that gets no room keeps its length, its tokens have no slot, and the layers give zeros for them) are what the layers take."""
         batch = self.lengths.shape[0]
         self.slots, positions, _, self.seqlens = paged_cache.reserve_pages(self.block_table, self.lengths, tokens, self.free_pages, self.num_free,
                                                                            self.page_block_size)
         self.positions, self.tree, self._before = positions.view(batch, tokens), None, self.lengths
+        # keys that the layers look at: none where there was no room, since the table names other sequences' pages there
+        self._attended = torch.where(self.seqlens > self._before, self.seqlens, 0)
         self.lengths = self.seqlens
 
     def begin_tree(self, parents: torch.Tensor):
         """Room for a tree of drafted tokens per sequence (parents: paged_cache.tree_layout), whose positions are their depths."""
         self.begin(parents.shape[1])
-        self.tree, self.positions = paged_cache.tree_layout(parents, self._before)
+        room = self.seqlens > self._before
+        self.tree, self.positions = paged_cache.tree_layout(torch.where(room[:, None], parents, -2), self._before)  # (without room: padding)
+        self._attended = torch.where(room, self._before, 0)
 
     def accept(self, path: torch.Tensor, nodes: int):
         """Keeps the accepted path of every tree of the step (paged_cache.keep_tree_path) and gives the other nodes' pages back.  A sequence that had no
@@ -184,9 +188,9 @@ class PagedSelfAttention(torch.nn.Module):
         q = rotary_axes_to_cache(q, k, v, emb._cos_cached, emb._sin_cached, positions, self.sections, params.slots, k_cache, v_cache, cycled=self.cycled,
                                  interleaved=emb.interleaved)
         if params.tree is not None:
-            return flash_attn_tree_with_kvcache(q, k_cache, v_cache, params.tree, params._before, block_table=params.block_table,
+            return flash_attn_tree_with_kvcache(q, k_cache, v_cache, params.tree, params._attended, block_table=params.block_table,
                                                 softmax_scale=self.softmax_scale)
-        return flash_attn_with_kvcache(q, k_cache, v_cache, cache_seqlens=params.seqlens, block_table=params.block_table, causal=True,
+        return flash_attn_with_kvcache(q, k_cache, v_cache, cache_seqlens=params._attended, block_table=params.block_table, causal=True,
                                        softmax_scale=self.softmax_scale)
 
 
