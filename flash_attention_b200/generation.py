@@ -140,15 +140,15 @@ class PagedInferenceParams:
                                                                            self.page_block_size)
         self.positions, self.tree, self._before = positions.view(batch, tokens), None, self.lengths
         # keys that the layers look at: none where there was no room, since the table names other sequences' pages there
-        self._attended = torch.where(self.seqlens > self._before, self.seqlens, 0)
+        self._room = self.seqlens > self._before
+        self._attended = torch.where(self._room, self.seqlens, 0)
         self.lengths = self.seqlens
 
     def begin_tree(self, parents: torch.Tensor):
         """Room for a tree of drafted tokens per sequence (parents: paged_cache.tree_layout), whose positions are their depths."""
         self.begin(parents.shape[1])
-        room = self.seqlens > self._before
-        self.tree, self.positions = paged_cache.tree_layout(torch.where(room[:, None], parents, -2), self._before)  # (without room: padding)
-        self._attended = torch.where(room, self._before, 0)
+        self.tree, self.positions = paged_cache.tree_layout(torch.where(self._room[:, None], parents, -2), self._before)  # (without room: padding)
+        self._attended = torch.where(self._room, self._before, 0)
 
     def accept(self, path: torch.Tensor, nodes: int):
         """Keeps the accepted path of every tree of the step (paged_cache.keep_tree_path) and gives the other nodes' pages back.  A sequence that had no

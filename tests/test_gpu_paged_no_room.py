@@ -33,8 +33,9 @@ def test_zeros(heads, heads_k, dim, tree, nodes):
     assert params.seqlens.tolist() == [64 + nodes, 64, 64]
     out, want = layer(*rows, params), layer(*[t[:1] for t in rows], alone)
     assert not out[1:].any() and want.any() and not torch.isnan(want).any()
-    # (parts of the keys may be cut differently: two roundings of bf16 results)
-    assert (out[:1].float() - want.float()).abs().max() <= 2 * torch.finfo(torch.bfloat16).eps * want.float().abs().max()
+    # (The keys may be cut into other parts.  Each side rounds the weights, whose sum is 1, and the result: two half steps of the largest value.)
+    largest = max(first[2].float().abs().max(), rows[2].float().abs().max())
+    assert (out[:1].float() - want.float()).abs().max() <= 2.1 * torch.finfo(torch.bfloat16).eps * largest
     own = params.block_table[0, 1].item()
     now = params.caches.clone()
     now[:, :, own], before[:, :, own] = 0, 0
@@ -42,11 +43,12 @@ def test_zeros(heads, heads_k, dim, tree, nodes):
     if tree:
         params.accept(torch.zeros(3, 1, dtype=torch.int32, device="cuda"), nodes)
         assert params.lengths.tolist() == [65, 64, 64]
-    # room again: the same sequences are served as if nothing had been
+    # two pages come free: the second sequence gets its turn, the third does not
     params.end(torch.tensor([True, False, False], device="cuda"))
     params.begin(1)
-    assert params.seqlens.tolist() == [1, 65, 65]
-    assert not torch.isnan(layer(*x(1), params)).any()
+    assert params.seqlens.tolist() == [1, 65, 64]
+    out = layer(*x(1), params)
+    assert out[:2].any(-1).all() and not torch.isnan(out).any() and not out[2].any()
 
 
 def test_a_table_that_is_full():
