@@ -170,7 +170,8 @@ class PagedSelfAttention(torch.nn.Module):
     forward(q, k, v, params, positions=None): q (batch, tokens, nheads, head_dim), k and v (batch, tokens, nheads_k, head_dim), fresh from the projections,
     of the tokens that params.begin or begin_tree made room for.  One launch turns q and k and stores k and v at their slots, then
     attention over the cache: causal, or by the tree.  positions: (axes, batch, tokens) where they are not the places in the sequence (images, video);
-    sections: pairs of each axis (apply_rotary_emb_axes), max_position: rows of the tables."""
+    sections: pairs of each axis (apply_rotary_emb_axes), max_position: rows of the tables, at least as many as a sequence's pages hold where its places
+    are its positions (tokens outside the tables are not turned)."""
 
     def __init__(self, layer_idx: int, head_dim: int, sections, max_position: int, softmax_scale=None, rotary_base=10000.0, cycled=False,
                  rotary_interleaved=False, device=None):
@@ -180,10 +181,13 @@ class PagedSelfAttention(torch.nn.Module):
         self.rotary_emb = RotaryEmbedding(2 * sum(self.sections), base=rotary_base, interleaved=rotary_interleaved, device=device)
 
     def forward(self, q, k, v, params: PagedInferenceParams, positions: Optional[torch.Tensor] = None):
+        if positions is None:
+            capacity = params.block_table.shape[1] * params.page_block_size
+            if self.max_position < capacity:
+                raise ValueError("PagedSelfAttention: max_position %d is less than the %d tokens that a sequence's pages hold" % (self.max_position, capacity))
+            positions = params.positions[None].expand(len(self.sections), -1, -1)
         emb = self.rotary_emb
         emb._update_cos_sin_cache(self.max_position, device=q.device, dtype=q.dtype)
-        if positions is None:
-            positions = params.positions[None].expand(len(self.sections), -1, -1)
         k_cache, v_cache = params.caches[self.layer_idx].unbind(0)
         q = rotary_axes_to_cache(q, k, v, emb._cos_cached, emb._sin_cached, positions, self.sections, params.slots, k_cache, v_cache, cycled=self.cycled,
                                  interleaved=emb.interleaved)
