@@ -342,6 +342,11 @@ void require_device(std::initializer_list<const Tensor*> ts) {
   }
 }
 
+// The calls have no forward-mode derivative: a tangent is refused, not lost
+void require_no_tangent(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) require(!t || !t->_fw_grad(0).defined(), "forward-mode derivatives are not supported");
+}
+
 // at::empty without the way through the dispatcher (a call has two to four results)
 Tensor fresh(c10::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
   return Tensor(at::detail::empty_cuda(sizes, type, dev, std::nullopt));
@@ -418,6 +423,7 @@ py::tuple tree_fwd(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const
   }
   require(num_splits >= 0 && num_splits <= 128, "num_splits must be in [0, 128]");
   require(fits({batch, batch_c, cap, nodes, heads, heads / heads_k * nodes, batch * heads * nodes}), "sizes are out of range");
+  require_no_tangent({&q_in, &kc, &vc, maybe(k_in), maybe(v_in)});
   require_device({&q_in, &kc, &vc, &mask, &lens, maybe(k_in), maybe(v_in), maybe(table), maybe(batch_idx)});
   require(direct(kc, true) && direct(vc, true), "k_cache / v_cache must be 16-byte aligned, with contiguous last dimension and strides that are multiples of 8");
   if (k_in)  // (what is written must not be one element in several places)
@@ -542,6 +548,7 @@ std::pair<Tensor, Tensor> turn_axes(const Tensor& q_in, const MaybeTensor& k_in,
     require(!inplace || (q_in.stride(-1) == 1 && !repeats(q_in) && (slots || !*t || ((*t)->stride(-1) == 1 && !repeats(**t)))),
             "in-place rotation needs a unit stride in the last dimension and elements of its own");
   require(fits({tokens, heads, heads_k, cos_in.size(0)}), "sizes are out of range");
+  require_no_tangent({&q_in, maybe(k_in), maybe(v_in), &cos_in, &sin_in, maybe(k_cache), maybe(v_cache)});
   require_device({&q_in, maybe(k_in), maybe(v_in), &cos_in, &sin_in, &positions, maybe(slots), maybe(k_cache), maybe(v_cache)});
 
   const c10::cuda::CUDAGuard guard(q_in.device());

@@ -208,6 +208,7 @@ def apply_rotary_emb_axes(q, k, cos, sin, positions, sections, cycled=False, int
         take turns (axis a > 0 has pairs a, a + axes, ..., as many as its section; the first axis has what is left).
     interleaved: pairs are (even, odd) dimensions instead of (first half, second half).
     inplace: q and k are overwritten and returned; not where a gradient is needed.
+    Gradients of q and k, of any order, backwards; tensors with a tangent (torch.autograd.forward_ad) are refused.
 
     Returns (q, k)."""
     return _glue().rotary_axes(q, k, cos, sin, positions, sections, cycled, interleaved, inplace)

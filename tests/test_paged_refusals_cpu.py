@@ -41,3 +41,24 @@ def test_rotary_tables_shorter_than_a_sequences_pages():
         call(192)
     with pytest.raises(RuntimeError, match="CUDA"):  # positions of the caller's own
         call(191, positions=i32(1, 2, 5))
+
+
+def test_tangents_are_refused_not_lost():
+    """A dual tensor of forward-mode differentiation does not require a gradient; the calls would give a result without a tangent."""
+    import torch.autograd.forward_ad as fwd
+
+    import flash_attention_b200 as fa
+    from flash_attention_b200.layers.rotary import apply_rotary_emb_axes, rotary_axes_to_cache
+
+    turn = dict(q=half(2, 7, 4, 64), k=half(2, 7, 2, 64), cos=half(30, 32), sin=half(30, 32), positions=i32(1, 2, 7), sections=(32,))
+    store = dict(v=half(2, 7, 2, 64), slots=torch.zeros(14, dtype=torch.int64), k_cache=half(5, 16, 2, 64), v_cache=half(5, 16, 2, 64))
+    tree = dict(q=half(2, 5, 4, 64), k_cache=half(2, 32, 2, 64), v_cache=half(2, 32, 2, 64), tree_mask=i32(2, 5, 1), cache_seqlens=i32(2))
+    with fwd.dual_level():
+        for name, call, args in [(n, apply_rotary_emb_axes, turn) for n in ("q", "k", "cos", "sin")] + [(n, rotary_axes_to_cache, {**turn, **store}) for n in "qkv"] + [
+                (n, fa.flash_attn_tree_with_kvcache, tree) for n in ("q", "k_cache", "v_cache")]:
+            for needs in (False, True):  # with a gradient as well
+                dual = fwd.make_dual(args[name].clone().requires_grad_(needs), torch.ones_like(args[name]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(**{**args, name: dual})
+        with pytest.raises(RuntimeError, match="CUDA"):  # nothing wrong but the device
+            apply_rotary_emb_axes(**turn)
