@@ -347,6 +347,14 @@ void require_no_tangent(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) require(!t || !t->_fw_grad(0).defined(), "forward-mode derivatives are not supported");
 }
 
+// Written in place: autograd then refuses to use a value that it saved before
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // (inference tensors have no version, and are never saved)
+}
+void refuse_gradients_in_place(std::initializer_list<const Tensor*> ts, const char* what) {
+  for (const Tensor* t : ts) require(!t || !at::GradMode::is_enabled() || !t->requires_grad(), what, ": in place only where no gradient is needed");
+}
+
 // at::empty without the way through the dispatcher (a call has two to four results)
 Tensor fresh(c10::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
   return Tensor(at::detail::empty_cuda(sizes, type, dev, std::nullopt));
@@ -466,6 +474,7 @@ py::tuple tree_fwd(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const
     status = fa_fwd_tree(&t, st);
   }
   check(status, "flash_attn_tree_with_kvcache");
+  if (k_in) changed(kc), changed(vc);
   return py::make_tuple(out, lse);
 }
 
@@ -586,6 +595,9 @@ std::pair<Tensor, Tensor> turn_axes(const Tensor& q_in, const MaybeTensor& k_in,
     status = fa_rotary_axes(&a, st);
   }
   check(status, slots ? "rotary_axes_to_cache" : "apply_rotary_emb_axes");
+  if (inplace) changed(q_in);
+  if (inplace && k_in && !slots) changed(*k_in);
+  if (slots) changed(*k_cache), changed(*v_cache);
   return {q_out, k_out};
 }
 
@@ -624,7 +636,7 @@ py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::non
 py::tuple rotary_axes(const Tensor& q, const MaybeTensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions, const std::vector<int64_t>& sections,
                       bool cycled, bool interleaved, bool inplace) {
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad()))) {
-    require(!inplace, "apply_rotary_emb_axes: in place only where no gradient is needed");
+    if (inplace) refuse_gradients_in_place({&q, maybe(k)}, "apply_rotary_emb_axes");
     const auto r = TurnNode::apply(q, k, cos, sin, positions, sections, cycled, interleaved, false);
     return py::make_tuple(r[0], k ? py::cast(r[1]) : py::none());
   }
@@ -636,6 +648,7 @@ py::tuple rotary_axes(const Tensor& q, const MaybeTensor& k, const Tensor& cos, 
 Tensor rotary_to_cache(const Tensor& q, const MaybeTensor& k, const MaybeTensor& v, const Tensor& cos, const Tensor& sin, const Tensor& positions,
                        const std::vector<int64_t>& sections, bool cycled, bool interleaved, bool inplace, const Tensor& slots, const MaybeTensor& k_cache,
                        const MaybeTensor& v_cache) {
+  if (inplace) refuse_gradients_in_place({&q}, "rotary_axes_to_cache");
   return turn_axes(q, k, v, {cos, sin, positions, sections, cycled, interleaved, false}, inplace, slots, k_cache, v_cache).first;
 }
 
@@ -668,6 +681,7 @@ py::tuple reserve_pages(const Tensor& table, const Tensor& lens, const MaybeTens
   a.free_pages = i32(free_pages), a.pool = free_pages.size(0), a.num_free = i32(num_free);
   a.slots = static_cast<int64_t*>(slots.data_ptr()), a.positions = i32(positions), a.cu_seqlens = i32(cu), a.seqlens = i32(seqlens), a.total = total;
   check(fa_reserve_pages(&a, stream_of(table)), "reserve_pages");
+  changed(table), changed(num_free);
   return py::make_tuple(slots, positions, cu, seqlens);
 }
 
@@ -679,6 +693,7 @@ void release_pages(const Tensor& table, const Tensor& lens, const Tensor& keep, 
   check(fa_release_pages(i32(table), table.stride(0), table.size(0), table.size(1), page, i32(lens), i32(keep), i32(free_pages), free_pages.size(0),
                          i32(num_free), stream_of(table)),
         "release_pages");
+  changed(free_pages), changed(num_free);
 }
 
 // tree_layout: (words, positions)
@@ -778,6 +793,9 @@ Tensor keep_path(const py::object& given, const Tensor& lens, const Tensor& path
   if (table) a.block_table = i32(*table), a.table_stride = table->stride(0), a.page_block_size = page > 0 ? page : 1;
   a.path = i32(path), a.path_stride = path.stride(0), a.depth = path.size(1), a.nodes = nodes;
   check(fa_keep_path(&a, stream_of(lens)), "keep_tree_path");
+  if (at && some) changed(first);
+  if (!at)
+    for (size_t i = 0; i < ptrs.size(); ++i) changed(THPVariable_Unpack(PySequence_Fast_ITEMS(given.ptr())[i]));
   return out;
 }
 

@@ -62,3 +62,18 @@ def test_tangents_are_refused_not_lost():
                     call(**{**args, name: dual})
         with pytest.raises(RuntimeError, match="CUDA"):  # nothing wrong but the device
             apply_rotary_emb_axes(**turn)
+
+
+def test_in_place_to_cache_refuses_gradients():
+    from flash_attention_b200.layers.rotary import rotary_axes_to_cache
+
+    args = dict(k=half(2, 7, 2, 64), v=half(2, 7, 2, 64), cos=half(30, 32), sin=half(30, 32), positions=i32(1, 2, 7), sections=(32,),
+                slots=torch.zeros(14, dtype=torch.int64), k_cache=half(5, 16, 2, 64), v_cache=half(5, 16, 2, 64))
+    q = half(2, 7, 4, 64).requires_grad_(True)
+    for x in (q, q * 1):
+        with pytest.raises(RuntimeError, match="gradient"):
+            rotary_axes_to_cache(x, inplace=True, **args)
+    with pytest.raises(RuntimeError, match="CUDA"):  # nothing else is wrong without gradients, or out of place
+        rotary_axes_to_cache(q, **args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        rotary_axes_to_cache(q, inplace=True, **args)
