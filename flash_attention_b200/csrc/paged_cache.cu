@@ -322,6 +322,11 @@ __global__ void __launch_bounds__(128) keep_path_kernel(const __grid_constant__ 
   }
 }
 
+// The limit of 48 KB without this counts a kernel's static shared memory as well
+int plan_smem_limit(fa_host::DeviceOnce& once, const void* kernel, int bytes, const char* name) {
+  return bytes > 40 * 1024 ? fa_host::raise_smem_limit(once, kernel, 224 * 1024, name) : 0;
+}
+
 template <typename V>
 int launch_keep(const FaKeepArgs& a, cudaStream_t st) {
   KeepParams p;
@@ -333,8 +338,7 @@ int launch_keep(const FaKeepArgs& a, cudaStream_t st) {
   p.pieces = per_head * a.heads_k;
   const int smem = a.depth * 16;
   static fa_host::DeviceOnce once;
-  if (smem > 48 * 1024)
-    if (int rc = fa_host::raise_smem_limit(once, reinterpret_cast<const void*>(&keep_path_kernel<V>), 200 * 1024, "keep_path_kernel")) return rc;
+  if (int rc = plan_smem_limit(once, reinterpret_cast<const void*>(&keep_path_kernel<V>), smem, "keep_path_kernel")) return rc;
   for (int c0 = 0; c0 < a.n_caches || c0 == 0; c0 += kKeepCaches) {
     const int n = a.n_caches - c0 < kKeepCaches ? a.n_caches - c0 : kKeepCaches;
     for (int i = 0; i < n; ++i) p.caches[i] = a.caches[c0 + i];
@@ -345,10 +349,6 @@ int launch_keep(const FaKeepArgs& a, cudaStream_t st) {
     if (int rc = fa_host::check_launch("keep_path_kernel")) return rc;
   }
   return 0;
-}
-
-int plan_smem_limit(fa_host::DeviceOnce& once, const void* kernel, int bytes, const char* name) {
-  return bytes > 40 * 1024 ? fa_host::raise_smem_limit(once, kernel, 224 * 1024, name) : 0;
 }
 
 }  // namespace

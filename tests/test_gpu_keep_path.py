@@ -100,3 +100,18 @@ def test_a_sequence_that_had_no_room_leaves_the_others_pages_alone():
     want = c.clone()
     want[3, 60:64], want[4, :4] = k[0, :4], k[0, 4:]
     assert torch.equal(kc, want) and torch.equal(vc, want)
+
+
+@pytest.mark.parametrize("dim", [8, 6])  # in pieces of 16 bytes, and of two
+@pytest.mark.parametrize("depth", [2560, 2561, 3071, 3073, 12288])
+def test_the_longest_paths(depth, dim):
+    """Around the shared memory that a launch has without asking, and the most there may be."""
+    c = cache(1, 2 * depth + 5, 1, dim)
+    was = c.clone()
+    path = torch.arange(1, 2 * depth, 2, device="cuda").int()[None]
+    assert pc.keep_tree_path([c], ints([3]), path, 2 * depth).tolist() == [3 + depth]
+    want = was.clone()
+    want[0, 3:3 + depth] = was[0, 4:4 + 2 * depth:2]
+    assert torch.equal(c, want)
+    with pytest.raises(RuntimeError, match="12288"):
+        pc.keep_tree_path([c], ints([3]), torch.zeros(1, 12289, dtype=torch.int32, device="cuda"), 2 * depth)
