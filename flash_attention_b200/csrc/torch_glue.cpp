@@ -403,13 +403,13 @@ py::tuple tree_fwd(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const
   require(d > 0 && d <= 256 && d % 8 == 0, "head dimension must be a multiple of 8, at most 256");
   require(heads_k > 0 && heads > 0 && heads % heads_k == 0, "Number of heads in key/value must divide number of heads in query");
   require(is_type(mask, at::kInt, 3) && mask.size(1) == nodes && mask.size(2) == (nodes + 31) / 32 && (mask.size(0) == batch || mask.size(0) == 1) &&
-              mask.stride(2) == 1,
+              (mask.size(2) == 1 || mask.stride(2) == 1),
           "the tree mask must be int32 words of shape (batch or 1, nodes, ceil(nodes / 32)) with contiguous last dimension");
   require(is_type(lens, at::kInt, 1) && lens.size(0) == batch && lens.is_contiguous(), "cache_seqlens must be int32, contiguous, one per sequence");
   int64_t cap = kc.size(1), page = 0;
   if (table) {
     require(!batch_idx, "Paged KVcache does not support cache_batch_idx");
-    require(is_type(*table, at::kInt, 2) && table->size(0) == batch && table->stride(1) == 1,
+    require(is_type(*table, at::kInt, 2) && table->size(0) == batch && (table->size(1) <= 1 || table->stride(1) == 1),
             "block_table must be int32 of shape (batch, pages per sequence) with contiguous last dimension");
     require(cap % 64 == 0 && cap > 0, "Paged KV cache block size must be divisible by 64");
     page = cap;

@@ -77,3 +77,17 @@ def test_in_place_to_cache_refuses_gradients():
         rotary_axes_to_cache(q, **args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         rotary_axes_to_cache(q, inplace=True, **args)
+
+
+def test_one_column_may_have_any_stride():
+    """A last dimension of one entry is contiguous whatever its stride says, which for a slice of a transposed tensor is not 1."""
+    import flash_attention_b200 as fa
+
+    args = dict(q=half(2, 5, 4, 64), k_cache=half(6, 64, 2, 64), v_cache=half(6, 64, 2, 64), cache_seqlens=i32(2))
+    table, words = i32(3, 2).t()[:, :1], i32(1, 2, 5).permute(1, 2, 0)
+    assert table.is_contiguous() and table.stride(1) != 1 and words.stride(2) != 1
+    for kw in (dict(tree_mask=words), dict(tree_mask=i32(2, 5, 1), block_table=table), dict(tree_mask=words, block_table=table)):
+        with pytest.raises(RuntimeError, match="CUDA"):  # nothing wrong but the device
+            fa.flash_attn_tree_with_kvcache(**args, **kw)
+    with pytest.raises(RuntimeError, match="words"):
+        fa.flash_attn_tree_with_kvcache(**{**args, "q": half(2, 40, 4, 64)}, tree_mask=i32(2, 2, 40).transpose(1, 2))
