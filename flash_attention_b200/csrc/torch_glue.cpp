@@ -342,6 +342,11 @@ void require_device(std::initializer_list<const Tensor*> ts) {
   }
 }
 
+// Two tensors of which a call writes one must not start at the same place (one given twice)
+void require_two(const Tensor& x, const Tensor& y, const char* what) {
+  require(x.numel() == 0 || y.numel() == 0 || x.data_ptr() != y.data_ptr(), what, ": the same tensor is given twice");
+}
+
 // The calls have no forward-mode derivative: a tangent is refused, not lost
 void require_no_tangent(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) require(!t || !t->_fw_grad(0).defined(), "forward-mode derivatives are not supported");
@@ -428,6 +433,7 @@ py::tuple tree_fwd(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const
     require(has_shape(*k_in, {batch, nodes, heads_k, d}) && has_shape(*v_in, {batch, nodes, heads_k, d}),
             "k and v must have shape (batch, nodes, nheads_k, headdim)");
     require(nodes <= cap, "the tree has more nodes than the KV cache has rows");
+    require_two(kc, vc, "k_cache and v_cache");
   }
   require(num_splits >= 0 && num_splits <= 128, "num_splits must be in [0, 128]");
   require(fits({batch, batch_c, cap, nodes, heads, heads / heads_k * nodes, batch * heads * nodes}), "sizes are out of range");
@@ -556,6 +562,9 @@ std::pair<Tensor, Tensor> turn_axes(const Tensor& q_in, const MaybeTensor& k_in,
   for (const MaybeTensor* t : {&k_in})
     require(!inplace || (q_in.stride(-1) == 1 && !repeats(q_in) && (slots || !*t || ((*t)->stride(-1) == 1 && !repeats(**t)))),
             "in-place rotation needs a unit stride in the last dimension and elements of its own");
+  if (inplace && k_in) require_two(q_in, *k_in, "q and k in place");
+  if (inplace && v_in) require_two(q_in, *v_in, "q and v in place");
+  if (slots) require_two(*k_cache, *v_cache, "k_cache and v_cache");
   require(fits({tokens, heads, heads_k, cos_in.size(0)}), "sizes are out of range");
   require_no_tangent({&q_in, maybe(k_in), maybe(v_in), &cos_in, &sin_in, maybe(k_cache), maybe(v_cache)});
   require_device({&q_in, maybe(k_in), maybe(v_in), &cos_in, &sin_in, &positions, maybe(slots), maybe(k_cache), maybe(v_cache)});

@@ -91,3 +91,30 @@ def test_one_column_may_have_any_stride():
             fa.flash_attn_tree_with_kvcache(**args, **kw)
     with pytest.raises(RuntimeError, match="words"):
         fa.flash_attn_tree_with_kvcache(**{**args, "q": half(2, 40, 4, 64)}, tree_mask=i32(2, 2, 40).transpose(1, 2))
+
+
+def test_one_tensor_for_two_that_are_written():
+    """Turned twice or not, K or V: which came last would decide."""
+    import flash_attention_b200 as fa
+    from flash_attention_b200.layers.rotary import apply_rotary_emb_axes, rotary_axes_to_cache
+
+    x, c = half(2, 7, 2, 64), half(5, 16, 2, 64)
+    turn = dict(cos=half(30, 32), sin=half(30, 32), positions=i32(1, 2, 7), sections=(32,))
+    with pytest.raises(RuntimeError, match="twice"):
+        apply_rotary_emb_axes(x, x, inplace=True, **turn)
+    with pytest.raises(RuntimeError, match="CUDA"):  # out of place it is only read
+        apply_rotary_emb_axes(x, x, **turn)
+    store = dict(slots=torch.zeros(14, dtype=torch.int64), k_cache=c)
+    with pytest.raises(RuntimeError, match="twice"):
+        rotary_axes_to_cache(x, x, x, v_cache=c, **store, **turn)
+    for k, v in ((x, x.clone()), (x.clone(), x)):  # read while q is written
+        with pytest.raises(RuntimeError, match="twice"):
+            rotary_axes_to_cache(x, k, v, v_cache=c.clone(), inplace=True, **store, **turn)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        rotary_axes_to_cache(x, x, x, v_cache=c.clone(), **store, **turn)
+    tree = dict(q=half(2, 5, 4, 64), tree_mask=i32(2, 5, 1), cache_seqlens=i32(2), k_cache=half(2, 32, 2, 64))
+    new = dict(k=half(2, 5, 2, 64), v=half(2, 5, 2, 64))
+    with pytest.raises(RuntimeError, match="twice"):
+        fa.flash_attn_tree_with_kvcache(**tree, v_cache=tree["k_cache"], **new)
+    with pytest.raises(RuntimeError, match="CUDA"):  # only read
+        fa.flash_attn_tree_with_kvcache(**tree, v_cache=tree["k_cache"])
