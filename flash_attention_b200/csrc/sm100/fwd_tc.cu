@@ -805,10 +805,11 @@ int launch_fwd_tc(const FaFwdArgs& a, int64_t kv_batches, const TreeCall* tree, 
   const int n_m = (a.seqlen_q + NT * P.tile_pos - 1) / (NT * P.tile_pos);
   dim3 grid(n_m * P.num_splits, a.heads / P.pack, a.batch);
   if (tree) {
-    // the model's constants: 5 us for what a CTA does outside its blocks, 2.1 for a block of two tiles, 3 for one of two CTAs that share an SM, 2.25 for 64 keys at head
-    // dims above 128 (per block from 2048 to 4096 keys, one part, all SMs: 2.1, 3.3, 2.1)
+    // the model's constants: 5 us for what a CTA does outside its blocks, 2.1 for a block of 128 keys of two tiles, 3 for one of two CTAs that share an SM, 3 at head dims
+    // above 128 (per block from 2048 to 4096 keys, one part, all SMs: 2.1, 3.3, and at head dims 136, 160, 192, 256 2.4, 2.8, 3.0, 3.3; 1.9 to 2.6 on a fifth of the
+    // SMs.  With 2.25 there 32 sequences of 100 to 6000 keys, 40 nodes, 8/2 heads of 256 took 106.5 us, 98.3 with 3; 30 other shapes the same)
     const double part_bytes = (double)P.pack * a.seqlen_q / n_m * a.head_dim * 8;  // (written and read again)
-    P.plan = fa_host::part_plan(5.f, C::CTAS == 2 ? 3.f : NT == 2 ? 2.1f : 2.25f, part_bytes, a.batch, (int64_t)grid.y * n_m, fa_host::sm_count() * C::CTAS,
+    P.plan = fa_host::part_plan(5.f, C::CTAS == 2 ? 3.f : NT == 2 ? 2.1f : 3.f, part_bytes, a.batch, (int64_t)grid.y * n_m, fa_host::sm_count() * C::CTAS,
                                 P.num_splits);
     grid = dim3(P.plan.ctas);
   }
@@ -909,7 +910,7 @@ int fwd_tc_tree_parts(const FaFwdArgs& a) {
   const int pack = pack_heads(a.heads / a.heads_k), tile_pos = kBM / pack, tiles = a.head_dim > 128 || tree_one_tile(a) ? 1 : 2;
   const int64_t row_blocks = (a.seqlen_q + tiles * tile_pos - 1) / (tiles * tile_pos);
   const int slots = fa_host::sm_count() * (a.head_dim <= 128 && tiles == 1 ? 2 : 1);
-  return fa_host::tree_parts(a.batch, a.heads / pack * row_blocks, slots, a.seqlen_k, kBN, a.head_dim > 128 ? 2.25 : 1.6);
+  return fa_host::tree_parts(a.batch, a.heads / pack * row_blocks, slots, a.seqlen_k, kBN, a.head_dim > 128 ? 3.0 : 1.6);
 }
 
 static volatile int g_last_tiles = 0;
