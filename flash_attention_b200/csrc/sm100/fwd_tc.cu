@@ -808,6 +808,8 @@ int launch_fwd_tc(const FaFwdArgs& a, int64_t kv_batches, const TreeCall* tree, 
     // the model's constants: 5 us for what a CTA does outside its blocks, 2.1 for a block of 128 keys of two tiles, 3 for one of two CTAs that share an SM, 3 at head dims
     // above 128 (per block from 2048 to 4096 keys, one part, all SMs: 2.1, 3.3, and at head dims 136, 160, 192, 256 2.4, 2.8, 3.0, 3.3; 1.9 to 2.6 on a fifth of the
     // SMs.  With 2.25 there 32 sequences of 100 to 6000 keys, 40 nodes, 8/2 heads of 256 took 106.5 us, 98.3 with 3; 30 other shapes the same)
+    // The 5 us are fitted to whole calls: with the 7.3 that a CTA with one block takes outside it, that case took 106.5 instead of 96.3, 50 trees of 64 nodes, 7 to
+    // 5802 keys, 4 heads of 32 69.6 instead of 73.7, 62 other shapes the same.
     const double part_bytes = (double)P.pack * a.seqlen_q / n_m * a.head_dim * 8;  // (written and read again)
     P.plan = fa_host::part_plan(5.f, C::CTAS == 2 ? 3.f : NT == 2 ? 2.1f : 3.f, part_bytes, a.batch, (int64_t)grid.y * n_m, fa_host::sm_count() * C::CTAS,
                                 P.num_splits);
