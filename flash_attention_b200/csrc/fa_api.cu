@@ -551,8 +551,10 @@ int fa_fwd_tree(const FaTreeArgs* t, fa_stream_t stream) {
   if (splits < 0) return 1;
   const FaKvcacheArgs& a = t->kv;
   if (check_tensor(a.q, "q") || check_tensor(a.kcache, "kcache") || check_tensor(a.vcache, "vcache") || check_tensor(a.out, "out")) return 1;
+  if (a.knew.ptr && (check_tensor(a.knew, "knew") || check_tensor(a.vnew, "vnew"))) return 1;  // (stored in 16-byte pieces)
   FA_REQUIRE(a.softmax_lse != nullptr, "softmax_lse: null pointer");
   FA_REQUIRE(splits == 1 || (a.lse_accum && a.out_accum), "split-KV needs lse_accum and out_accum");
+  FA_REQUIRE(splits == 1 || (reinterpret_cast<uintptr_t>(a.out_accum) & 15) == 0, "out_accum: pointer must be 16-byte aligned");
   if (refuse_if_device_failed()) return 3;
   const TreePath path = tree_path(a);
   const bool more = splits > 1, prep = a.knew.ptr != nullptr && path == kTreeGeneric;  // (the others store the nodes themselves)

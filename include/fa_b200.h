@@ -259,7 +259,7 @@ int fa_rotary(const FaRotaryArgs* args, fa_stream_t stream);
 
 /* Attention of the nodes of a tree of drafted tokens.  kv describes the call as for fa_fwd_kvcache with seqlen_q = nodes per
    sequence: cache_seqlens (required) counts the tokens in front of the tree, and node j's key and value are row cache_seqlens[b] + j of
-   the cache: put there by this call when knew / vnew are given (seqlen_new = seqlen_q), else already there.  Node i sees every key in front of the
+   the cache: put there by this call when knew / vnew are given (seqlen_new = seqlen_q; pointers and strides as for q), else already there.  Node i sees every key in front of the
    tree, and node j iff bit j % 32 of mask[b * mask_stride_b + i * mask_stride_s + j / 32] is set.  (strides in words, 0 to share a mask;
    a row holds (seqlen_q + 31) / 32 words)  Windows must be open (-1) and the rotary fields unset.  A node that sees no key gives out = 0 and
    softmax_lse = +inf.  Entries of block_table or cache_batch_idx that name no page or slot of the cache read as zeros and are not written. */

@@ -118,3 +118,29 @@ def test_one_tensor_for_two_that_are_written():
         fa.flash_attn_tree_with_kvcache(**tree, v_cache=tree["k_cache"], **new)
     with pytest.raises(RuntimeError, match="CUDA"):  # only read
         fa.flash_attn_tree_with_kvcache(**tree, v_cache=tree["k_cache"])
+
+
+def test_c_entry_of_trees_refuses_rows_that_are_not_aligned(lib):
+    """The kernels store new keys and values, and partial results, in 16-byte pieces."""
+    import ctypes
+
+    from flash_attention_b200 import _lib
+
+    def tree(**kw):
+        t = _lib.FaTreeArgs()
+        a = t.kv
+        a.batch = a.batch_cache = 2
+        a.seqlen_q = a.seqlen_new = 5
+        a.seqlen_cache, a.heads, a.heads_k, a.head_dim, a.dtype = 64, 4, 2, 64, 1
+        a.window_left = a.window_right = -1
+        a.cache_seqlens = a.softmax_lse = t.mask = 4096
+        for name in ("q", "kcache", "vcache", "out", "knew", "vnew"):
+            setattr(a, name, _lib.FaTensor(kw.get(name, 4096), kw.get(name + "_stride", 64 * 320), 128, 64))
+        for name in ("num_splits", "lse_accum", "out_accum"):
+            setattr(a, name, kw.get(name, 0))
+        return lib.fa_fwd_tree(ctypes.byref(t), ctypes.c_void_p()), lib.fa_last_error()
+
+    for kw, message in ((dict(knew=4098), b"knew: pointer"), (dict(vnew=4104), b"vnew: pointer"), (dict(knew_stride=1001), b"knew: strides"),
+                        (dict(vnew=None), b"value"), (dict(num_splits=2, lse_accum=4096, out_accum=4100), b"out_accum: pointer")):
+        rc, err = tree(**kw)
+        assert rc == 1 and message in err, (kw, err)
