@@ -121,7 +121,8 @@ class PagedInferenceParams:
 
     caches: (layers, 2, pages, page_block_size, nheads_k, head_dim), K at [:, 0]; block_table: (batch, pages per sequence) int32; lengths: (batch,)
     int32, tokens in the cache.  A step is begin() or begin_tree(), the layers, and for a tree accept().  Nothing is read back, so a step of one size
-    can be captured in a CUDA graph."""
+    can be captured in a CUDA graph.  A replay starts from the tensor that `lengths` was when the capture began and leaves the new lengths in another: end the
+    captured step by copying them there."""
 
     def __init__(self, layers: int, batch: int, pages: int, pages_per_sequence: int, page_block_size: int, nheads_k: int, head_dim: int, dtype, device):
         self.page_block_size = page_block_size
@@ -130,7 +131,7 @@ class PagedInferenceParams:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(pages, dtype=torch.int32, device=device)
         self.num_free = torch.tensor([pages, 0], dtype=torch.int32, device=device)
-        self.slots = self.positions = self.seqlens = self.tree = None
+        self.slots = self.positions = self.seqlens = self.tree = self._before = None
 
     def begin(self, tokens: int):
         """Room for `tokens` more tokens of every sequence.  slots, positions (batch, tokens) and seqlens (the lengths with them; a sequence
@@ -152,16 +153,18 @@ class PagedInferenceParams:
 
     def accept(self, path: torch.Tensor, nodes: int):
         """Keeps the accepted path of every tree of the step (paged_cache.keep_tree_path) and gives the other nodes' pages back.  A sequence that had no
-        room for its tree keeps nothing of it."""
+        room for its tree keeps nothing of it.  Once a step, and not after end()."""
+        if self._before is None:  # (pages would go back twice)
+            raise ValueError("accept: no step has begun, or it has been accepted or ended")
         kept = paged_cache.keep_tree_path(self.caches.flatten(0, 1), self._before, path, nodes, block_table=self.block_table, seqlens=self.seqlens)
         paged_cache.release_pages(self.block_table, self.seqlens, kept, self.free_pages, self.num_free, self.page_block_size)
-        self.lengths = kept
+        self.lengths, self._before = kept, None
 
     def end(self, ended: torch.Tensor):
         """Sequences where ended (batch,) is true give all their pages back and start from nothing."""
         keep = torch.where(ended, 0, self.lengths)
         paged_cache.release_pages(self.block_table, self.lengths, keep, self.free_pages, self.num_free, self.page_block_size)
-        self.lengths = keep
+        self.lengths, self._before = keep, None
 
 
 class PagedSelfAttention(torch.nn.Module):

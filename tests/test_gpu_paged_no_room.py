@@ -1,4 +1,4 @@
-"""PagedSelfAttention for sequences that got no room: zeros, whatever their tables name, and the other sequences as if they were alone."""
+"""PagedSelfAttention for sequences that got no room: zeros, whatever their tables name, and the other sequences as if they were alone.  Pages go back once."""
 import pytest
 import torch
 
@@ -65,3 +65,24 @@ def test_a_table_that_is_full():
     assert params.seqlens.tolist() == [100, 30] and not out[0].any() and out[1].any(-1).all()
     params.accept(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), 30)
     assert params.lengths.tolist() == [100, 1]
+
+
+def test_a_step_is_accepted_once():
+    """A second accept, or one behind end(), would put the same pages on the stack again."""
+    params = PagedInferenceParams(1, 2, 10, 4, 64, 2, 64, torch.bfloat16, "cuda")
+    path = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    parents = torch.arange(-1, 69, dtype=torch.int32, device="cuda").expand(2, -1)
+    for after in (lambda: params.accept(path, 70), lambda: params.end(torch.tensor([True, False], device="cuda"))):
+        params.begin_tree(parents)
+        assert params.num_free[0] < 8
+        after()
+        lengths, num = params.lengths.tolist(), params.num_free.tolist()
+        with pytest.raises(ValueError, match="accept"):
+            params.accept(path, 70)
+        assert params.lengths.tolist() == lengths and params.num_free.tolist() == num
+    stack = params.free_pages[: params.num_free[0]].tolist()
+    assert len(set(stack)) == len(stack)
+    # a chain of drafts after begin() is accepted like a tree
+    params.begin(3)
+    params.accept(torch.tensor([[0, 1], [0, -1]], dtype=torch.int32, device="cuda"), 3)
+    assert params.lengths.tolist() == [lengths[0] + 2, lengths[1] + 1]

@@ -144,3 +144,11 @@ def test_c_entry_of_trees_refuses_rows_that_are_not_aligned(lib):
                         (dict(vnew=None), b"value"), (dict(num_splits=2, lse_accum=4096, out_accum=4100), b"out_accum: pointer")):
         rc, err = tree(**kw)
         assert rc == 1 and message in err, (kw, err)
+
+
+def test_nothing_to_accept():
+    from flash_attention_b200.generation import PagedInferenceParams
+
+    params = PagedInferenceParams(1, 2, pages=8, pages_per_sequence=3, page_block_size=64, nheads_k=2, head_dim=64, dtype=torch.bfloat16, device="cpu")
+    with pytest.raises(ValueError, match="accept: no step"):
+        params.accept(i32(2, 3), 5)
