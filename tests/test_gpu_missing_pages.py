@@ -78,3 +78,31 @@ def test_lengths_past_the_capacity(heads, heads_k, dim, path, splits):
         x[GUARD + int(table[2, 0]), 10], x[GUARD + int(table[3, 2]), 63] = new[2, 0].cuda(), new[3, 0].cuda()
         assert torch.equal(w, x)
     check(out, lse, q, kc, vc, lens, block_table=table)
+
+
+@pytest.mark.parametrize("heads,heads_k,dim,path", [(4, 2, 128, "kvcache_prep+decode"), (16, 2, 64, "kvcache_prep+fwd_tc"), (4, 2, 40, "kvcache_prep+fwd_generic")])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_several_tokens(heads, heads_k, dim, path, splits):
+    """Five tokens, some of them in a page that is there and some not; a row of the table that names nothing, as for a sequence that had no room."""
+    g = torch.Generator().manual_seed(dim)
+    whole = [guarded(PAGE, heads_k, dim, g) for _ in range(2)]
+    was = [w.clone() for w in whole]
+    kc, vc = (w[GUARD:GUARD + POOL] for w in whole)
+    lens = torch.tensor([62, 126, 100, 190], dtype=torch.int32)  # the last runs past the capacity
+    table = torch.tensor([[3, -1, 5], [7, POOL, 0], [-1, -1, -1], [1, 2, 4]], dtype=torch.int32)
+    q = torch.randn(BATCH, 5, heads, dim, generator=g).bfloat16()
+    k, v = (torch.randn(BATCH, 5, heads_k, dim, generator=g).bfloat16() for _ in range(2))
+    out, lse = fa.flash_attn_with_kvcache(q.cuda(), kc, vc, k.cuda(), v.cuda(), cache_seqlens=lens.cuda(), causal=False, num_splits=splits, return_softmax_lse=True,
+                                          block_table=table.cuda())
+    assert _lib.last_path().startswith(path), _lib.last_path()
+    for w, x, new in zip(whole, was, (k, v)):
+        for b in range(BATCH):
+            for i in range(5):
+                row = int(lens[b]) + i
+                page = int(table[b, row // PAGE]) if row < 3 * PAGE else -1
+                if 0 <= page < POOL:
+                    x[GUARD + page, row % PAGE] = new[b, i].cuda()
+        assert torch.equal(w, x)
+    o, l, to, tl = TO.tree_attention(q, kc.cpu(), vc.cpu(), torch.ones(1, 5, 5, dtype=torch.bool), lens, block_table=table)
+    assert ((out.double().cpu() - o).abs() <= to).all()
+    assert ((lse.double().cpu() - l).abs() <= tl).all()
